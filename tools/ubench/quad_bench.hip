@@ -117,20 +117,18 @@ int main(int argc, char** argv) {
     unsigned long long* tl; CK(hipMalloc(&tl, (size_t)grid_b * 16 * 8)); CK(hipMemset(tl, 0, (size_t)grid_b * 16 * 8));
     CK(hipMemcpyToSymbol(HIP_SYMBOL(jst_qtl_base), &tl, sizeof(tl)));
 #endif
-    const char* only = getenv("QB_ONLY");  // "a": the pipelined kernel alone, "b": the quad kernel alone (fault isolation)
-    const bool run_a = !only || only[0] == 'a', run_b = !only || only[0] == 'b';
-    if (run_a) ka<<<grid_a, 512, lds_a, st>>>(L, W, pro, epi_a);
+    ka<<<grid_a, 512, lds_a, st>>>(L, W, pro, epi_a);
     CK(hipGetLastError());
     CK(hipStreamSynchronize(st));
     printf("[%s] pipe ran\n", name); fflush(stdout);
-    if (run_b) kb<<<grid_b, 256, lds_b, st>>>(L, W, pro, epi_b, sched);
+    kb<<<grid_b, 256, lds_b, st>>>(L, W, pro, epi_b, sched);
     CK(hipGetLastError());
     CK(hipStreamSynchronize(st));
     printf("[%s] quad ran\n", name); fflush(stdout);
     // clocks: the first milliseconds of a fresh process run far below the sustained clock
     for (int r = 0; r < (getenv("QB_WARM") ? atoi(getenv("QB_WARM")) : 300); ++r) {
-        if (run_a) ka<<<grid_a, 512, lds_a, st>>>(L, W, pro, epi_a);
-        if (run_b) kb<<<grid_b, 256, lds_b, st>>>(L, W, pro, epi_b, sched);
+        ka<<<grid_a, 512, lds_a, st>>>(L, W, pro, epi_a);
+        kb<<<grid_b, 256, lds_b, st>>>(L, W, pro, epi_b, sched);
     }
     CK(hipStreamSynchronize(st));
     {
@@ -193,10 +191,10 @@ int main(int argc, char** argv) {
     for (auto& e : ev) CK(hipEventCreate(&e));
     for (int r = 0; r < reps; ++r) {
         CK(hipEventRecord(ev[4 * r + 0], st));
-        if (run_a) ka<<<grid_a, 512, lds_a, st>>>(L, W, pro, epi_a);
+        ka<<<grid_a, 512, lds_a, st>>>(L, W, pro, epi_a);
         CK(hipEventRecord(ev[4 * r + 1], st));
         CK(hipEventRecord(ev[4 * r + 2], st));
-        if (run_b) kb<<<grid_b, 256, lds_b, st>>>(L, W, pro, epi_b, sched);
+        kb<<<grid_b, 256, lds_b, st>>>(L, W, pro, epi_b, sched);
         CK(hipEventRecord(ev[4 * r + 3], st));
     }
     CK(hipStreamSynchronize(st));
