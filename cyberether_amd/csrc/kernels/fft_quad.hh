@@ -44,10 +44,12 @@
 //   * transforms are handed out DYNAMICALLY.  With the static round robin (transform t to workgroup t mod grid) the 1024
 //     workgroups of a 16384-transform launch start over 12 us (the dispatcher), run at visibly different speeds and end
 //     between 132 and 171 us: 15 % of the grid x time rectangle is workgroups that have not started or have already
-//     finished (profiles/r05_experiments/g_workgroup_lifetimes.log).  A workgroup takes transform `blockIdx` first and
-//     every further one from a device counter (one scalar atomic per transform, issued by wavefront 0 in front of the
-//     wait for its LDS-DMA pieces and handed to the other wavefronts through an LDS word behind a barrier that is there
-//     anyway); the last workgroup out re-arms the counters for the next launch;
+//     finished (profiles/r05_experiments/g_workgroup_lifetimes.log).  So the last quarter of a long launch's rounds is
+//     claimed: one lane asks a device counter (an ordinary vector atomic) at the top of a transform for the one after it
+//     and hands the answer to the other wavefronts through an LDS word behind pass 2, 6000 ticks later, in front of a
+//     barrier that is there anyway.  Nobody waits for the answer at once: it retires behind the previous epilogue's
+//     stores, and asked for behind them with the wait next to it, it cost a launch 173 -> 226 us (h_dynamic_first.log).
+//     The last workgroup out re-arms the counters for the next launch;
 //   * everything else is the pipelined kernel's: persistent workgroups, resident window taps and pass-0 twiddles, small
 //     twiddle tables in LDS, LDS-only barriers, wave priorities, the epilogue functors and their cache policies.
 //
@@ -82,13 +84,6 @@ static_assert(4 * ((fft_quad_lds_bytes() + 1279) / 1280) * 1280 <= 160 * 1024, "
 #ifndef JST_QUAD_STATIC_NUM  // share of a launch's rounds handed out statically (see fft_quad_body)
 #define JST_QUAD_STATIC_NUM 3
 #define JST_QUAD_STATIC_DEN 4
-#endif
-// A workgroup whose claim counter has run out tries the partner counters (see fft_quad_body).  Measured, same box, three
-// alternating runs (tools/ubench/run_r05p.sh, profiles/r05_experiments/p_claim_stealing.log): 162.5-165.4 us against
-// 163.6-165.2 without -- the eight shares end 6 us apart either way, and what remains of the tail is the last transform of
-// every workgroup.  Off.
-#ifndef JST_QUAD_STEAL
-#define JST_QUAD_STEAL 0
 #endif
 #ifndef JST_QUAD_SPREAD  // outputs between two LDS-DMA pieces in the epilogue (0: all nine back to back in front of it)
 #define JST_QUAD_SPREAD 1
@@ -160,19 +155,6 @@ __device__ __forceinline__ quad_v4u quad_row_rsrc(const void* row, uint32_t byte
 // sched: kQuadSchedWords zeroed U32 words of device memory owned by the caller (eight claim counters and the count of finished
 // workgroups, kQuadSchedStride words = 256 bytes apart), or null for the static round robin.
 constexpr uint32_t kQuadSchedStride = 64, kQuadSchedWords = 9 * kQuadSchedStride;
-// The next unclaimed transform, asked for by ONE wavefront of the workgroup: a SCALAR atomic (one request per wavefront, the
-// answer in an SGPR, counted by lgkmcnt -- not queued behind the epilogue's stores in vmcnt order) issued in front of the
-// wait for the wavefront's own LDS-DMA pieces, so that the two waits overlap; request and wait are ONE statement (between
-// two statements hipcc may spill the destination SGPR -- this kernel spills ~40 -- before the answer has arrived).  Through
-// `__hip_atomic_fetch_add` the answer came back behind `s_waitcnt vmcnt(0)`, i.e. behind every store of the previous
-// epilogue: 173 -> 226 us per launch (profiles/r05_experiments/h_dynamic_first.log).
-template <int VMCNT>
-__device__ __forceinline__ uint32_t quad_claim_and_wait(uint32_t* counter) {
-    uint32_t v = 1u;
-    __asm__ volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt vmcnt(%2)\n\ts_waitcnt lgkmcnt(0)" : "+s"(v) : "s"(counter), "n"(VMCNT) : "memory");
-    return v;
-}
-
 template <bool FWD, class Pro, class Epi>
 __device__ __forceinline__ void fft_quad_body(const FftLayout& L, const float2* __restrict__ W, const Pro& pro,
                                               const Epi& epi_arg, const uint32_t bid, const uint32_t grid, uint32_t* sched) {
@@ -187,7 +169,8 @@ __device__ __forceinline__ void fft_quad_body(const FftLayout& L, const float2* 
     typedef __attribute__((address_space(3))) unsigned char* lds_bytes_t;
     float2* twl = reinterpret_cast<float2*>(smem_raw);
     float2* data = twl + kQuadTwEntries;  // 4032 bytes in: 16-byte aligned
-    volatile uint32_t* handover = reinterpret_cast<volatile uint32_t*>(data + kQuadDataElems);
+    typedef volatile __attribute__((address_space(3))) uint32_t* lds_u32_t;
+    const lds_u32_t handover = (lds_u32_t)reinterpret_cast<uint32_t*>(data + kQuadDataElems);
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -210,7 +193,6 @@ __device__ __forceinline__ void fft_quad_body(const FftLayout& L, const float2* 
     uint32_t t = bid;
     const uint32_t total = (uint32_t)L.transforms;  // < 2^31 (the launcher checks)
     if (t >= total) return;
-    // the transform after this one: static round robin, or the next one nobody has taken (wavefront 0 asks, see below)
     // The first `srounds` rounds are the static round robin, the rest is claimed one transform at a time -- from EIGHT counters
     // (workgroup b uses counter b mod 8, which hands out the transforms = b mod 8 of the claimed region; the dispatcher
     // deals workgroups to the eight XCDs in that order, so a counter's clients are one XCD's).  Atomics on one address are
@@ -220,7 +202,6 @@ __device__ __forceinline__ void fft_quad_body(const FftLayout& L, const float2* 
     // workgroups' speeds have drifted apart.
     const uint32_t srounds = sched ? (total / grid) * JST_QUAD_STATIC_NUM / JST_QUAD_STATIC_DEN : 0xffffffffu;
     uint32_t rnd = 0;  // round of the transform in hand
-    uint32_t fetched = t + grid;
     int64_t in_base, out_base;
     quad_bases(L, t, in_base, out_base);
     float2 opnd[16];  // element e = 8 j + b of this thread: position (tid + 256 j) + 512 b
@@ -253,11 +234,8 @@ __device__ __forceinline__ void fft_quad_body(const FftLayout& L, const float2* 
     // through the whole transform, and at 128 VGPRs two of the piece offsets then went to scratch -- with `s_waitcnt
     // vmcnt(0)` in front of their reloads, in the middle of the epilogue's stores.
     const bool young = bid >= (grid >> 1);
-    // the first transform's pieces: everything issued so far (window taps, twiddles, pieces, the counter's answer) has landed
-    uint32_t home = bid & 7u;  // the claim counter this workgroup asks (its own share first)
-    if (wv == 0 && 1u >= srounds) fetched = srounds * grid + 8u * quad_claim_and_wait<0>(sched + kQuadSchedStride * home) + home;
-    else JST_WAIT_VMCNT(0);
-    if (tid == 0) *handover = fetched;
+    // the first transform's pieces: everything issued so far (window taps, twiddles, pieces) has landed
+    JST_WAIT_VMCNT(0);
 #ifdef JST_QUAD_TIMELINE
     unsigned long long qacc[12] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}, qlast = clock64(), qiters = 0;
     const unsigned long long qwall0 = wall_clock64();
@@ -276,13 +254,16 @@ __device__ __forceinline__ void fft_quad_body(const FftLayout& L, const float2* 
         __builtin_amdgcn_s_setprio(JST_QUAD_PRIO_PASS);
         lds_barrier();
         JST_QSTAMP(0);  // top barrier
-        // which transform comes next (wavefront 0 left it in the hand-over word in front of the barrier), and -- wavefront 0, a
-        // whole transform ahead -- which one after that
-        const uint32_t tn = (uint32_t)__builtin_amdgcn_readfirstlane((int)*handover);
-        const bool more = tn < total;
-        int64_t nin = 0, nout = 0;
-        quad_bases(L, more ? tn : t, nin, nout);
-        fetched = tn + grid;
+        // which transform comes next: the static one, or -- asked for here, used behind pass 2 -- the next unclaimed one of this
+        // workgroup's counter.  The opaque zero makes the address a per-lane one: for a uniform address the compiler broadcasts
+        // the answer to the wavefront and waits for it on the spot.  Nothing may be computed from it up here, for the same reason.
+        const bool claim = rnd + 1u >= srounds;
+        uint32_t claimed = 0u;
+        if (claim && tid == 0) {
+            uint32_t zero = 0u;
+            __asm__ volatile("" : "+v"(zero));
+            claimed = __hip_atomic_fetch_add(sched + kQuadSchedStride * (bid & 7u) + zero, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
         // ---- pass 0: in place, Multiply applied on the way in ---------------------------------------------------------------
         // (all passes: BOTH butterflies' operands are requested before the first is computed -- their slots are disjoint, and a
         // pass is then one LDS round trip deep instead of two)
@@ -354,7 +335,13 @@ __device__ __forceinline__ void fft_quad_body(const FftLayout& L, const float2* 
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int b = 0; b < 8; ++b) z[j][b] = quad_lds_read(p3 + 32 * j + b);
+        // the word's last readers were in the transform before this one: at least four barriers ago
+        if (claim && tid == 0) *handover = claimed;
         lds_barrier();
+        const uint32_t tn = claim ? srounds * grid + 8u * (uint32_t)__builtin_amdgcn_readfirstlane((int)*handover) + (bid & 7u) : t + grid;
+        const bool more = tn < total;
+        int64_t nin = 0, nout = 0;
+        quad_bases(L, more ? tn : t, nin, nout);
         JST_QSTAMP(7);  // pass-3 reads + the barrier behind them
         const quad_v4u r_next = quad_row_rsrc(pro.row(nin), (uint32_t)N * 8u);
         if constexpr (JST_QUAD_SPREAD == 0) {
@@ -408,29 +395,10 @@ __device__ __forceinline__ void fft_quad_body(const FftLayout& L, const float2* 
         // it (tools/check_quad_isa.py counts them in the ISA)
         constexpr int kAfter = JST_QUAD_SPREAD == 0 ? 16 : 16 - (8 * JST_QUAD_SPREAD + 1);
         static_assert(kAfter >= 0, "nine pieces inside sixteen outputs");
-        // ... and, wavefront 0, the transform after the next (the other wavefronts read the word behind the next barrier, and read
-        // it last behind the top barrier of THIS transform, four barriers ago)
-        ++rnd;  // the round of transform tn; `fetched` (tn + grid so far) is for round rnd + 1
-        if (wv == 0 && rnd + 1u >= srounds) {
-            fetched = srounds * grid + 8u * quad_claim_and_wait<kAfter * STORES>(sched + kQuadSchedStride * home) + home;
-#if JST_QUAD_STEAL
-            // this counter's share is handed out: look at the partner counters (b ^ 4, then ^ 2, then ^ 1: the eight shares
-            // end pairwise, then in fours, then together) and stay with the first that still has work
-            for (uint32_t hop = 4u; fetched >= total && hop != 0u; hop >>= 1) {
-                const uint32_t other = home ^ hop;
-                const uint32_t got = srounds * grid + 8u * quad_claim_and_wait<63>(sched + kQuadSchedStride * other) + other;
-                if (got < total) {
-                    fetched = got;
-                    home = other;
-                }
-            }
-#endif
-        } else {
-            JST_WAIT_VMCNT(kAfter * STORES);
-        }
+        JST_WAIT_VMCNT(kAfter * STORES);
         JST_QSTAMP(10);  // own pieces landed
-        if (tid == 0) *handover = fetched;
         t = tn;
+        ++rnd;
         out_base = nout;
     }
     if (sched && tid == 0) {
