@@ -91,39 +91,6 @@ __global__ __launch_bounds__(1024) void k(float* out, float seed, int iters) {
     out[blockIdx.x * 1024 + threadIdx.x] = s;
 }
 
-// packed forms: 8 register pairs
-typedef float v2f __attribute__((ext_vector_type(2)));
-#define R8(OP) OP("%0", "%8") OP("%1", "%9") OP("%2", "%10") OP("%3", "%11") OP("%4", "%12") OP("%5", "%13") OP("%6", "%14") OP("%7", "%15")
-#define P_ADD_VV(d, s) "v_pk_add_f32 " d ", " d ", " s "\n"
-#define P_MUL_VV(d, s) "v_pk_mul_f32 " d ", " d ", " s "\n"
-#define P_ADD_SV(d, s) "v_pk_add_f32 " d ", %16, " d "\n"
-#define P_FMA_VVV(d, s) "v_pk_fma_f32 " d ", " d ", " s ", " s "\n"
-#define P_ADD_NEG(d, s) "v_pk_add_f32 " d ", " d ", " s " neg_lo:[0,1] neg_hi:[0,1]\n"
-#define P_ADD_SWZ(d, s) "v_pk_add_f32 " d ", " d ", " s " op_sel:[0,1] op_sel_hi:[1,0]\n"
-template <int FORM>
-__global__ __launch_bounds__(1024) void kp(float* out, float seed, int iters) {
-    v2f a[8], b[8];
-    for (int i = 0; i < 8; ++i) { a[i] = v2f{seed + threadIdx.x + i, seed + i}; b[i] = v2f{seed * 0.5f + i, seed}; }
-    typedef int v2i __attribute__((ext_vector_type(2)));
-    const v2i sc = v2i{__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, seed * 1.0000001f)),
-                       __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, seed))};
-    for (int it = 0; it < iters; ++it) {
-#define PBODY(OPS)                                                                                                   \
-    asm volatile(R8(OPS) R8(OPS) R8(OPS) R8(OPS)                                                                      \
-                 : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(a[7])     \
-                 : "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "v"(b[4]), "v"(b[5]), "v"(b[6]), "v"(b[7]), "s"(sc))
-        if (FORM == 0) PBODY(P_ADD_VV);
-        if (FORM == 1) PBODY(P_MUL_VV);
-        if (FORM == 2) PBODY(P_ADD_SV);
-        if (FORM == 3) PBODY(P_FMA_VVV);
-        if (FORM == 4) PBODY(P_ADD_NEG);
-        if (FORM == 5) PBODY(P_ADD_SWZ);
-    }
-    v2f s = v2f{0, 0};
-    for (int i = 0; i < 8; ++i) s += a[i];
-    out[blockIdx.x * 1024 + threadIdx.x] = s.x + s.y;
-}
-
 template <class K>
 void run(const char* name, K kern, int waves_per_simd) {
     float* out; hipMalloc(&out, 256 * 1024 * 4);
@@ -173,12 +140,6 @@ int main() {
         run("v_sqrt_f32", k<10>, w);
         run("v_cvt_u32_f32", k<11>, w);
         run("v_mov_b32_dpp quad_perm", k<13>, w);
-        run("v_pk_add_f32 v,v,v", kp<0>, w);
-        run("v_pk_mul_f32 v,v,v", kp<1>, w);
-        run("v_pk_add_f32 v,s,v", kp<2>, w);
-        run("v_pk_fma_f32 v,v,v,v", kp<3>, w);
-        run("v_pk_add_f32 neg", kp<4>, w);
-        run("v_pk_add_f32 op_sel swz", kp<5>, w);
     }
     return 0;
 }
