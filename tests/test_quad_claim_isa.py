@@ -26,7 +26,8 @@ def test_the_claim_is_a_vector_atomic_nobody_waits_for_at_once(tmp_path):
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     out = tmp_path / "quad.s"
     csrc = os.path.join(ROOT, "cyberether_amd", "csrc")
-    subprocess.run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++20", "-ffp-contract=off", "-S", "--cuda-device-only",
+    subprocess.run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++20", "-ffp-contract=off", "-Xclang", "-target-feature",
+                    "-Xclang", "-packed-fp32-ops", "-S", "--cuda-device-only",
                     "-I", os.path.join(csrc, "kernels"), "-I", csrc, "-I", os.path.join(ROOT, "include"),
                     os.path.join(csrc, "kernels", "fft_side.hip"), "-o", str(out)], check=True, capture_output=True)
     r = check_quad_isa.check(out.read_text())

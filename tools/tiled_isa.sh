@@ -3,7 +3,7 @@
 # skeleton and the register counts.  Diagnostic.
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 cd $ROOT/cyberether_amd/csrc
-/opt/rocm/bin/hipcc -O3 -std=c++20 -fPIC -ffp-contract=off -fvisibility=hidden --offload-arch=gfx950 -D__HIP_PLATFORM_AMD__ $EXTRA --cuda-device-only -S kernels/${UNIT:-fft_tiled}.hip -o /tmp/unit.s 2>&1 | grep error -A5
+/opt/rocm/bin/hipcc -O3 -std=c++20 -fPIC -ffp-contract=off -fvisibility=hidden --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -D__HIP_PLATFORM_AMD__ $EXTRA --cuda-device-only -S kernels/${UNIT:-fft_tiled}.hip -o /tmp/unit.s 2>&1 | grep error -A5
 L=$(grep -n "^_ZN.*$1.*:" /tmp/unit.s | head -1 | cut -d: -f1)
 awk -v s=$L 'NR>=s' /tmp/unit.s > /tmp/k.s
 END=$(grep -n "s_endpgm" /tmp/k.s | head -1 | cut -d: -f1)

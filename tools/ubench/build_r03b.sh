@@ -4,7 +4,7 @@
 ROOT=$(cd "$(dirname "$0")/../.." && pwd)
 B=$ROOT/tools/ubench/bin
 mkdir -p $B
-HC="/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off -D__HIP_PLATFORM_AMD__ -I $ROOT/cyberether_amd/csrc/kernels -I $ROOT/cyberether_amd/csrc -I $ROOT/include"
+HC="/opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off -D__HIP_PLATFORM_AMD__ -I $ROOT/cyberether_amd/csrc/kernels -I $ROOT/cyberether_amd/csrc -I $ROOT/include"
 $HC $ROOT/tools/ubench/floor_bisect.hip -o $B/floor_bisect &
 $HC -DJST_FFT_TIMELINE $ROOT/tools/ubench/fft_timeline.hip -o $B/fft_timeline_r03 &
 for r in 0 1; do for l in 0 1; do

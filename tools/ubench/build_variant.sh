@@ -4,7 +4,7 @@
 ROOT=$(cd "$(dirname "$0")/../.." && pwd)
 NAME=$1; shift
 V=$ROOT/cyberether_amd/lib/variants; mkdir -p $V/obj_$NAME
-FLAGS="-O3 -std=c++20 -fPIC -ffp-contract=off -fvisibility=hidden --offload-arch=gfx950 -Wno-unused-function -Wno-unused-result -D__HIP_PLATFORM_AMD__"
+FLAGS="-O3 -std=c++20 -fPIC -ffp-contract=off -fvisibility=hidden --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-function -Wno-unused-result -D__HIP_PLATFORM_AMD__"
 cd $ROOT/cyberether_amd/csrc
 UNITS=${VARIANT_UNITS:-"fft_side fft_kernels"}   # translation units recompiled under the extra flags
 for f in $UNITS; do

@@ -2,7 +2,7 @@
 // the spectrogram's 256 tiles of cycle k-1 as 512-thread workgroups behind them (blockIdx >= 512): the spectrogram
 // workgroups are dispatched as the first spectrum workgroups of each CU retire, i.e. into the launch's tail.
 // Compared with the two kernels launched one after the other.  Diagnostic only.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off -I cyberether_amd/csrc/kernels -I cyberether_amd/csrc
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off -I cyberether_amd/csrc/kernels -I cyberether_amd/csrc
 //         tools/ubench/combined_bench.hip
 #include "../../cyberether_amd/csrc/kernels/spectrogram.hip"
 #include "fft_lds_r03_variants.hh"  // the round-3 header with its A/B switches (the product header dropped them)

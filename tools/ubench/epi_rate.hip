@@ -2,7 +2,7 @@
 // in registers, no memory traffic: ns per element per wavefront and per SIMD at 1, 2, 4, 8 wavefronts per SIMD.
 // Answers: what does the VALU really sustain on this instruction mix (literals, SGPR operands, transcendentals,
 // half-rate conversions) compared with the 1.1 ns per plain v_add/v_mul of valu_ops.hip?
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off -I cyberether_amd/csrc/kernels tools/ubench/epi_rate.hip
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off -I cyberether_amd/csrc/kernels tools/ubench/epi_rate.hip
 #include "device_math.hh"
 
 #include <cstdio>

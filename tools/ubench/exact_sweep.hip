@@ -7,7 +7,7 @@
 //   chain : amplitude_range_from_power (main path + bail-out) vs range_f32(amplitude_from_power) on all 2^32
 //           power bit patterns, for several (coeff, scale, offset) triples
 // Prints mismatch counts; exit code 0 only if the shipped configuration has none.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off [-DJST_DIV_EXPM1=div_v1 ...] \
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off [-DJST_DIV_EXPM1=div_v1 ...] \
 //         -I cyberether_amd/csrc/kernels tools/ubench/exact_sweep.hip -o exact_sweep
 #include "device_math.hh"
 

@@ -3,7 +3,7 @@
 // real window operand resident and the row-index side output.  Thread 0 of every workgroup stamps clock64 at the
 // phase boundaries of every transform into a ring of three iterations: what is read back are the LAST three
 // transforms of each workgroup (30, 31, 32 of 32: the last one has no successor to prefetch).  Diagnostic only.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off -DJST_FFT_TIMELINE -DJST_OPND_RESIDENT=1
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off -DJST_FFT_TIMELINE -DJST_OPND_RESIDENT=1
 //         -I cyberether_amd/csrc/kernels -I cyberether_amd/csrc -I include tools/ubench/fft_timeline_batched.hip
 #include "fft_lds.hh"
 #include <algorithm>

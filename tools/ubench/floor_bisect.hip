@@ -18,7 +18,7 @@
 // Every variant reports back-to-back launch time, the event-pair median, the spread of workgroup starts / ends
 // (s_memrealtime, one extra launch) and a permutation-invariant checksum of the output bits (all variants of one
 // WINDOW class must agree).
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off -I cyberether_amd/csrc/kernels -I cyberether_amd/csrc \
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off -I cyberether_amd/csrc/kernels -I cyberether_amd/csrc \
 //        tools/ubench/floor_bisect.hip -o tools/ubench/bin/floor_bisect
 #include "fft_lds_r03_variants.hh"  // the round-3 header with its A/B switches (the product header dropped them)
 

@@ -2,7 +2,7 @@
 // (1024 x 4096 cf32, tone + AWGN per row, Blackman x (-1)^n window, range -100..0 dB) over a ring of 16 input
 // slots (512 MiB > Infinity Cache), median/mean launch time by hipEvents and an order-independent checksum of
 // the output bits so that variants compiled with different -D switches can be compared bit for bit.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off [-DJST_...] -I cyberether_amd/csrc/kernels \
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off [-DJST_...] -I cyberether_amd/csrc/kernels \
 //         -I cyberether_amd/csrc tools/ubench/fused_bench.hip -o fused_bench_<variant>
 // Diagnostic only; the product path is cyberether_amd/lib/libjetstream_hip.so.
 #include "fft_lds_r03_variants.hh"  // the round-3 header with its A/B switches (the product header dropped them)

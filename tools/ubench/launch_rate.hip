@@ -1,7 +1,7 @@
 // How fast does the chip START wavefronts?  Empty workgroups (one store each) of W wavefronts with L bytes of LDS and a register
 // footprint of 64 / 128 VGPRs: grid / (event time - empty-launch time) = workgroups per microsecond.  Diagnostic (round 6: the
 // LDS-tiled FFT kernels' one-workgroup-per-tile launches run at this rate, not at their tiles' cost).
-//   hipcc --offload-arch=gfx950 -O3 tools/ubench/launch_rate.hip -o tools/ubench/bin/launch_rate
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/ubench/launch_rate.hip -o tools/ubench/bin/launch_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

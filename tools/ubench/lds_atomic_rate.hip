@@ -5,7 +5,7 @@
 //   2  random dword addresses in a 16 KiB histogram
 //   3  plain ds_write_b32 with pattern 0 (for scale)
 //   4  bank = 16 * (row & 1) + column (bin * 32 words pitch, two interleaved copies): deterministic two lanes per bank
-// hipcc --offload-arch=gfx950 -O3 -o bin/lds_atomic_rate lds_atomic_rate.hip
+// hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o bin/lds_atomic_rate lds_atomic_rate.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

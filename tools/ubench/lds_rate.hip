@@ -1,6 +1,6 @@
 // LDS instruction throughput per CU at 16 wavefronts per CU (the fused kernel's occupancy): ds_read_b64 vs ds_read2_b64,
 // ds_write_b64 vs ds_write2st64_b64, conflict-free addresses (lane-contiguous 8-byte elements).
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 tools/ubench/lds_rate.hip -o tools/ubench/bin/lds_rate
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 tools/ubench/lds_rate.hip -o tools/ubench/bin/lds_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

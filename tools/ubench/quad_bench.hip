@@ -2,7 +2,7 @@
 // 2 workgroups per CU) against fft_quad_kernel (fft_quad.hh, 256 threads, in-place exchange, rows by LDS-DMA, 4 workgroups per CU), both with
 // the product's functors (real window operand resident, provider fast, row-index side output) and cache policies.
 // Bit-compares every F32 value and every index byte of the two, then times them alternately over a 16-slot ring.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off [-DJST_QUAD_...] -I cyberether_amd/csrc/kernels \
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off [-DJST_QUAD_...] -I cyberether_amd/csrc/kernels \
 //         -I cyberether_amd/csrc -I include tools/ubench/quad_bench.hip -o tools/ubench/bin/quad_bench_<variant>
 // Diagnostic only; the product path is cyberether_amd/lib/libjetstream_hip.so.
 #define JST_LOAD_AUX 2

@@ -1,7 +1,7 @@
 // What does the memory system alone allow for the headline workload's traffic shape?  Reads 1024 x 4096 cf32
 // (32 MiB) and writes 1024 x 4096 f32 (16 MiB) with no arithmetic to speak of, in the launch shapes the FFT
 // kernels use.  The result is the practical floor for any fused multiply->fft->amplitude->range kernel.
-// Build: hipcc --offload-arch=gfx950 -O3 tools/ubench/stream_floor.hip -o tools/ubench/stream_floor
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/ubench/stream_floor.hip -o tools/ubench/stream_floor
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,6 +1,6 @@
 // Per-workgroup phase timeline of the LDS-tiled FFT kernels (columns / blocks) at SURVEY config 3's transform
 // (100 x 160000 points, pad fused in): wall-clock stamps by thread 0 of every workgroup.  Diagnostic only.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off -DJST_TILED_TIMELINE -I cyberether_amd/csrc/kernels
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off -DJST_TILED_TIMELINE -I cyberether_amd/csrc/kernels
 //         -I cyberether_amd/csrc tools/ubench/tiled_timeline.hip
 #include "../../cyberether_amd/csrc/kernels/fft_tiled.hip"
 

@@ -1,7 +1,7 @@
 // Phase timeline of ONE workgroup of the single-kernel tiled FFT at multi-fm.yml's Filter transform: 8 x 8050 points
 // (2*5*5*7*23, 8000 valid samples, pad fused in), fold epilogue with 2 heads and fold 805 -- 8 workgroups in all, so the
 // kernel's duration IS a workgroup's lifetime.  Diagnostic only.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off -DJST_TILED_TIMELINE -I cyberether_amd/csrc/kernels
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off -DJST_TILED_TIMELINE -I cyberether_amd/csrc/kernels
 //         -I cyberether_amd/csrc -I include tools/ubench/tiled_timeline_8050.hip
 #include "../../cyberether_amd/csrc/kernels/fft_tiled.hip"
 

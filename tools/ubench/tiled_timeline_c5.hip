@@ -1,6 +1,6 @@
 // Per-workgroup phase timeline of the LDS-tiled FFT kernels at BASELINE config 5 (B x 65536 points, window fused in, provider fast
 // epilogue): wall-clock stamps by thread 0 of every workgroup, for several static plans (lane counts).  Diagnostic only.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++20 -ffp-contract=off -DJST_TILED_TIMELINE -I cyberether_amd/csrc/kernels
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++20 -ffp-contract=off -DJST_TILED_TIMELINE -I cyberether_amd/csrc/kernels
 //         -I cyberether_amd/csrc tools/ubench/tiled_timeline_c5.hip -o tools/ubench/bin/tiled_timeline_c5
 #include "../../cyberether_amd/csrc/kernels/fft_tiled.hip"
 

@@ -1,5 +1,5 @@
 // Dependent-issue latency of VALU ops on gfx950: NCH independent chains per wave, W waves per SIMD.
-// Build: hipcc --offload-arch=gfx950 -O3 tools/ubench/valu_dep.hip -o tools/ubench/valu_dep
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/ubench/valu_dep.hip -o tools/ubench/valu_dep
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

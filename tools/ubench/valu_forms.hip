@@ -1,7 +1,7 @@
 // VALU throughput per SIMD on gfx950 by instruction FORM (operand kinds), W wavefronts per SIMD, 16 independent
 // destinations per wavefront (no dependency stalls): what does a wave64 instruction cost the SIMD when both sources
-// are VGPRs, when one is an SGPR, when it is packed, when it is an FMA ...
-// Build: hipcc --offload-arch=gfx950 -O3 tools/ubench/valu_forms.hip -o tools/ubench/bin/valu_forms
+// are VGPRs, when one is an SGPR, when it is an FMA ...
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/ubench/valu_forms.hip -o tools/ubench/bin/valu_forms
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

@@ -1,7 +1,7 @@
 // Per-opcode VALU throughput on gfx950: 32 independent instructions of ONE opcode per loop
 // iteration (inline asm, 8 independent register chains), 4 waves per SIMD on every SIMD.
 // Reports cycles per wave-instruction per SIMD at the measured shader clock (s_memtime vs wall).
-// Build: hipcc --offload-arch=gfx950 -O3 tools/ubench/valu_ops.hip -o tools/ubench/valu_ops
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/ubench/valu_ops.hip -o tools/ubench/valu_ops
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

@@ -1,5 +1,5 @@
 // VALU issue-rate microbenchmark for gfx950: scalar f32 add/mul vs packed (v_pk_*) vs fma,
-// 4 waves/SIMD, register-resident.  Build: hipcc --offload-arch=gfx950 -O3 -ffp-contract=off
+// 4 waves/SIMD, register-resident.  Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -ffp-contract=off
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef float v2f __attribute__((ext_vector_type(2)));
